@@ -415,7 +415,7 @@ __global__ __launch_bounds__ (512, 4) void olasave8k_kernel (const OlaParams p)
 // one dispatched first takes 7.5 us per block and the other 17.4 (the hardware serves the oldest wave first), the first ends its
 // run at 198 us and the second works on alone until 252 (tools/sv8_progress.py, profiles/r05_sv8_progress_static.json) -- 40
 // blocks/us over the launch against 48.5 in its steady state, whatever the run lengths.  Here a workgroup CLAIMS its next block
-// when it needs it: tools/gen/gen_olasave8k.py, Gen8kDyn (the claim protocol, the mailbox, why a scalar atomic).
+// when it needs it: tools/gen/gen_olasave8k.py, Gen8kDyn (the claim protocol, the mailbox, the ticket's place among the loads and stores).
 #define PROT_SV8_DYN_CAT_(a, b) PROT_SV8_DYN_##a##_##b
 #ifdef PROT_SV8_STAMPS
 #define PROT_SV8_DYN_OUT_ "+v"(sv8_acc)
@@ -543,7 +543,7 @@ __global__ __launch_bounds__ (512, 4) void olasave8k_dyn_kernel (const OlaParams
 		__syncthreads ();
 	}
 
-	// ---- the workgroup's first claim (thread 0; the generated loop makes the later ones, wave 0 with a scalar atomic): its XCD's
+	// ---- the workgroup's first claim (thread 0; the generated loop makes the later ones, lane 0 of wave 0): its XCD's
 	// region first, the next ones when that is empty
 	const int nb  = (int)p.dyn_nb;
 	const int per = (nb + 7) / 8;

@@ -19,7 +19,7 @@ from gen8k_core import Gen8k  # noqa: E402
 S_BLK = S(38)                       # the block being transformed (index among the launch's whole in-range blocks of this channel)
 S_NEXT = S(89)                      # the block after it, or 0xffffffff: none left
 S_CTRX = SP(90)                     # wave 0: address of the counter of the region it draws from
-S_TK = S(92)                        # wave 0: the ticket in flight / arrived
+S_TK = S(92)                        # wave 0: the ticket that has arrived
 S_XR = S(93)                        # wave 0: the region it draws from (0..7: one per XCD, its own first)
 S_TRIES, S_PER, S_NB = S(94), S(95), S(96)   # wave 0: regions left to try; blocks per region; blocks in all
 S_ADV = S_SV                        # byte offset from the current block to the next one (the table pointer is dead behind the prologue)
@@ -37,11 +37,12 @@ class Gen8kDyn(Gen8k):
     steady state, whatever the run lengths (1.0 : 1.0 ... 1.55 : 0.45 all measure the same).  Here every block is claimed when it is
     needed: the stream's whole in-range blocks are dealt out in eight contiguous regions, one per XCD (a block's context rows are
     the rows its predecessor's workgroup has just read: they hit in that XCD's L2), each behind a counter of its own; wave 0 of a
-    workgroup draws a ticket with a scalar atomic (s_atomic_add ... glc: wave-uniform, through the scalar cache, lgkmcnt) a block
-    ahead -- issued behind the last LDS read of block B, collected in front of the first LDS write of block B + 1, published through
-    a mailbox word in LDS in front of that block's second barrier and read by all eight waves behind it, in time for the prefetch of
-    block B + 2's rows -- and moves on to the next region when its own is exhausted.  All 16 rows of a block are loaded (nothing is
-    carried from block to block, so the odd-context "mixed row" is just an address), the dry rows are copied aside as before."""
+    workgroup draws a ticket a block ahead with a returning vector atomic of its lane 0 (vmcnt, in order with the row loads in front
+    of it and the output stores behind it) -- issued behind the last LDS read of block B, arrived where block B + 1 waits for its
+    rows, published through a mailbox word in LDS in front of that block's second barrier and read by all eight waves behind it, in
+    time for the prefetch of block B + 2's rows -- and moves on to the next region when its own is exhausted.  All 16 rows of a
+    block are loaded (nothing is carried from block to block, so the odd-context "mixed row" is just an address), the dry rows are
+    copied aside as before."""
 
     def __init__(self, HS, MODE, opts=(), kind="run"):
         assert kind == "run" and MODE != MODE_SWEEP
@@ -75,7 +76,7 @@ class Gen8kDyn(Gen8k):
         n += 4
         self.RHO = [VP(n)]
         n += 2
-        self.G_NX, self.VT = V(n), V(n + 1)          # gathered frames (lanes 0..15); mailbox value
+        self.G_NX, self.VT = V(n), V(n + 1)          # gathered frames (lanes 0..15); mailbox value, wave 0's ticket in flight
         n += 2
         (self.A_RZ, self.A_RZH, self.A_R1, self.A_CH, self.A_X2, self.A_TL, self.VOFF, self.VG) = [V(n + i) for i in range(8)]
         n += 8
@@ -113,28 +114,41 @@ class Gen8kDyn(Gen8k):
         P.restore(st)     # (what wave 0 alone has put in flight is not in the other waves' queues: the bookkeeping forgets it -- wave
         P.label(skip)     # 0's own waits become stricter by that much, nobody's laxer)
 
+    def draw(self):
+        """(inside if_wave0) lane 0 adds 1 to the region's counter; the old value, the ticket, comes back in lane 0 of VT.  VOFF is 0
+        in that lane, so it serves as the address offset."""
+        P = self.P
+        P.v_mov(self.VT, Lit(1))
+        P.exec_lane0()
+        st = P.fork()
+        P.global_atomic_add(self.VT, self.VOFF, self.VT, S_CTRX)
+        P.restore(st)     # (not in the other waves' queues; what waits for it says so itself)
+        P.exec_all()
+
     def claim_issue(self):
         """wave 0: draw the next ticket of the current region (if the block after this one exists: there is nothing to draw behind
-        the end).  Nothing waits for it here."""
+        the end).  Nothing waits for it here: VT is free from the mailbox read of a block to the collection in the next one."""
         P = self.P
         def body():
             none = self.label("L_ci")
             P.s_cmp_eq_u32(S_NEXT, Lit(NONE))
             P.s_cbranch_scc1(none)
-            P.s_mov(S_TK, Lit(1))
-            P.s_atomic_add(S_TK, S_CTRX)
+            self.draw()
             P.label(none)
         self.if_wave0(body)
 
     def claim_collect_publish(self):
-        """wave 0: the ticket has had a block's time to arrive; turn it into a block (or move on to the next region, or find that
-        nothing is left) and put the answer into the mailbox.  The LDS queue is empty here (the explicit wait is for the scalar
-        atomic alone) and the workgroup barrier that follows the first exchange's writes orders the mailbox for the readers."""
+        """wave 0: turn the ticket into a block (or move on to the next region, or find that nothing is left) and put the answer into
+        the mailbox.  The ticket was drawn in front of the HS output stores, so the top of the loop has waited for it together with
+        the rows; the wait here states that (it never parks: at most those HS stores are in flight).  The workgroup barrier that
+        follows the first exchange's writes orders the mailbox for the readers."""
         P = self.P
         def body():
             retry, valid, none, pub = [self.label(x) for x in ("L_cr", "L_cv", "L_cn", "L_cp")]
-            P.s_wait_lgkm0_here()
+            P.s_wait_vm_here(self.HS)
             P.label(retry)
+            P.v_readfirstlane(S_TK, self.VT)
+            P.s_nop(4)
             P.s_mul_i32(S_T[3], S_XR, S_PER)                    # first block of the region
             P.s_sub_u32(S_A0.lo, S_NB, S_T[3])
             P.s_min_u32(S_A0.lo, S_A0.lo, S_PER)                # its length ...
@@ -153,9 +167,8 @@ class Gen8kDyn(Gen8k):
             P.s_cselect(S_A0.lo, Lit(1024), Lit(0))
             P.s_sub_u32(S_CTRX.lo, S_CTRX.lo, S_A0.lo)
             P.s_subb_u32(S_CTRX.hi, S_CTRX.hi, Lit(0))
-            P.s_mov(S_TK, Lit(1))
-            P.s_atomic_add(S_TK, S_CTRX)
-            P.s_wait_lgkm0_here()
+            self.draw()
+            P.s_wait_vm_here(0)                                 # (once per region that runs out)
             P.s_branch(retry)
             P.label(valid)
             P.s_add_u32(S_NEXT, S_T[3], S_TK)
@@ -323,9 +336,9 @@ class Gen8kDyn(Gen8k):
         P.s_waitcnt(vmcnt=0)
         P.label("L_top")
         self.stamp(0)
-        # the next block's rows have arrived (its 16 row loads and the gather were issued in front of this block's HS stores);
-        # no LDS operation is in flight here (the last ones were the reads of the fourth exchange, all consumed), and the scalar
-        # atomic of wave 0 may be: lgkmcnt is not waited for
+        # the next block's rows have arrived (its 16 row loads and the gather were issued in front of this block's HS stores), and
+        # with them wave 0's ticket (drawn between the two); no LDS operation is in flight here (the last ones were the reads of the
+        # fourth exchange, all consumed)
         P.s_waitcnt(vmcnt=HS)
         P.reset_queues(vm_stores=HS)
         self.stamp(1)
@@ -421,8 +434,8 @@ class Gen8kDyn(Gen8k):
                 issue(j)
                 fold(j - 1)
             fold(3)
-        # every LDS read of the block has been consumed: from here to the next block's first exchange no wait counts lgkmcnt --
-        # the ticket of the block after next has that long to arrive
+        # every load of the prefetch has been issued (flush_pending) and none of the HS stores: the ticket of the block after next has
+        # the third inverse pass and the stores to arrive in, and the counted wait at the top of the loop covers it
         P.settle(self.D)
         self.claim_issue()
         P.comment("---- inverse pass 3")

@@ -133,7 +133,7 @@ class Prog:
             for x in getattr(i, "srcs", []):
                 regs |= self._regs(x)
             self._need(regs)
-            if i.op in ("gload2", "gload1"):
+            if i.op in ("gload2", "gload1", "gatomic_add"):
                 self.vmq.append(self._regs(i.d))
             elif i.op == "gstore2":
                 self.vmq.append(set())
@@ -143,9 +143,6 @@ class Prog:
                 self.lgq.append(self._regs(i.d))
             elif i.op in ("ds_write_b64", "ds_write_b32"):
                 self.lgq.append(set())
-            # (s_atomic_add is NOT counted: scalar memory returns out of order with LDS, so a count that leaned on its position
-            # could be satisfied with the LDS operation in front of it still in flight; a wait computed from the LDS operations
-            # alone is at worst stricter than needed while the atomic is out.  Its result is waited for with an explicit lgkmcnt(0).)
         elif i.op == "s_waitcnt":
             if i.vmcnt is not None: del self.vmq[:max(0, len(self.vmq) - i.vmcnt)]
             if i.lgkmcnt is not None: del self.lgq[:max(0, len(self.lgq) - i.lgkmcnt)]
@@ -235,10 +232,10 @@ class Prog:
     def s_mul_hi_i32(self, d, a, b): return self.add(Ins("s_mul_hi_i32", "s_mul_hi_i32 %r, %r, %r" % (d, a, b), d=d, a=a, b=b))
     def s_and_b32(self, d, a, b): return self.add(Ins("s_and_b32", "s_and_b32 %r, %r, %r" % (d, a, b), d=d, a=a, b=b))
     def s_min_u32(self, d, a, b): return self.add(Ins("s_min_u32", "s_min_u32 %r, %r, %r" % (d, a, b), d=d, a=a, b=b))
-    def s_atomic_add(self, d, sbase):
-        """d (holding the addend) <- the 32-bit word at sbase before the add (glc: a wave-uniform fetch-and-add through the scalar
-        cache; returns through lgkmcnt, OUT of order with LDS operations: only lgkmcnt(0) says it has arrived)"""
-        return self.add(Ins("s_atomic_add", "s_atomic_add %r, %r, 0x0 glc" % (d, sbase), d=d, sbase=sbase))
+    def global_atomic_add(self, d, voff, data, sbase):
+        """d <- the 32-bit word at sbase + voff before `data` is added to it, per active lane (sc0: the old value comes back through
+        vmcnt, in order with the loads and stores around it)"""
+        return self.add(Ins("gatomic_add", "global_atomic_add %r, %r, %r, %r sc0" % (d, voff, data, sbase), d=d, voff=voff, data=data, sbase=sbase))
     def ds_write_b32(self, addr, data, off=0):
         assert 0 <= off < 65536
         return self.add(Ins("ds_write_b32", "ds_write_b32 %r, %r%s" % (addr, data, " offset:%d" % off if off else ""), addr=addr, data=data, off=off))
@@ -257,10 +254,11 @@ class Prog:
             assert 0 <= lgkmcnt <= 15
             parts.append("lgkmcnt(%d)" % lgkmcnt)
         return self.add(Ins("s_waitcnt", "s_waitcnt " + " ".join(parts), vmcnt=vmcnt, lgkmcnt=lgkmcnt))
-    def s_wait_lgkm0_here(self):
-        """an explicit `s_waitcnt lgkmcnt(0)` inside a region only some waves execute (a scalar atomic's result): seen by the emulator,
-        not by the generator's own wait bookkeeping (which describes every wave) nor by assert_no_waits_since"""
-        return self.add(Ins("s_waitcnt_x", "s_waitcnt lgkmcnt(0)", vmcnt=None, lgkmcnt=0))
+    def s_wait_vm_here(self, n):
+        """an explicit `s_waitcnt vmcnt(n)` inside a region only some waves execute (a ticket's arrival): seen by the emulator, not by
+        the generator's own wait bookkeeping (which describes every wave) nor by assert_no_waits_since"""
+        assert 0 <= n <= 63
+        return self.add(Ins("s_waitcnt_x", "s_waitcnt vmcnt(%d)" % n, vmcnt=n, lgkmcnt=None))
     def s_barrier(self): return self.add(Ins("s_barrier", "s_barrier"))
     def s_nop(self, n=0): return self.add(Ins("s_nop", "s_nop %d" % n))
     def s_setprio(self, n): return self.add(Ins("s_nop", "s_setprio %d" % n))
@@ -330,7 +328,6 @@ class _Wave:
         self.recent = []                    # VGPRs written by the last two VALU instructions (DPP hazard: 2 wait states)
         self.sgpr_wr = 99                   # instructions since a VALU wrote an SGPR (v_readlane / v_readfirstlane)
         self.done = False
-        self.smem_regs = set()              # SGPRs a scalar atomic in flight will write
 
 
 class Emu:
@@ -451,8 +448,6 @@ class Emu:
             raise TypeError(x)
 
         def srd(x):
-            if isinstance(x, S) and x.n in W_.smem_regs:
-                raise RuntimeError("s%d is read while the scalar atomic that writes it is in flight (no lgkmcnt(0) since)" % x.n)
             if isinstance(x, S): return int(s[x.n])
             if isinstance(x, Lit): return int(x.bits())
             if isinstance(x, (int, np.integer)): return int(x) & 0xffffffff
@@ -660,18 +655,7 @@ class Emu:
                 if i.vmcnt is not None:
                     while len(W_.vm_q) > i.vmcnt: W_.vm_q.pop(0)
                 if i.lgkmcnt is not None:
-                    # (scalar memory returns out of order with LDS: with one in flight only lgkmcnt(0) guarantees anything about IT;
-                    # the LDS operations in front of the allowed count are complete either way -- an smem entry is kept at the
-                    # queue's end until a wait for zero)
-                    if i.lgkmcnt == 0:
-                        W_.lgkm_q.clear()
-                        W_.smem_regs.clear()
-                    else:
-                        # the case that matters for safety: the atomic has already returned, so only LDS operations hold the count
-                        lds_q = [x for x in W_.lgkm_q if x[0] != "smem"]
-                        n_sm = len(W_.lgkm_q) - len(lds_q)
-                        while len(lds_q) > i.lgkmcnt: lds_q.pop(0)
-                        W_.lgkm_q = lds_q + [("smem", [])] * n_sm
+                    while len(W_.lgkm_q) > i.lgkmcnt: W_.lgkm_q.pop(0)
             elif op == "s_mov":
                 s[i.d.n] = srd(i.a)
             elif op == "s_mov64":
@@ -706,17 +690,21 @@ class Emu:
                 a, b = srd(i.a), srd(i.b)
                 s[i.d.n] = min(a, b)
                 W_.scc = int(a <= b)
-            elif op == "s_atomic_add":
+            elif op == "gatomic_add":
                 # (the waves of the emulated workgroup run one after the other: the read-modify-write is atomic by construction;
                 # `atomic_stride` > 1 stands for the other workgroups of a launch that draw from the same counter in between)
+                touch(regs_of(i.voff) + regs_of(i.data), regs_of(i.d), i.text)
                 base = srd(i.sbase.lo) | (srd(i.sbase.hi) << 32)
-                b0, arr = self._region(base)
-                wd = (base - b0) // 4
-                old = int(arr[wd])
-                arr[wd] = (old + srd(i.d) * getattr(self, "atomic_stride", 1)) & 0xffffffff
-                s[i.d.n] = old
-                W_.smem_regs.add(i.d.n)
-                W_.lgkm_q.append(("smem", []))
+                voff, data = rd32(i.voff), rd32(i.data)
+                for lane in np.flatnonzero(W_.exec):
+                    addr = base + int(voff[lane])
+                    b0, arr = self._region(addr)
+                    assert addr % 4 == 0, "atomic address"
+                    wd = (addr - b0) // 4
+                    old = int(arr[wd])
+                    arr[wd] = (old + int(data[lane]) * getattr(self, "atomic_stride", 1)) & 0xffffffff
+                    v[i.d.n][lane] = old
+                W_.vm_q.append(("load", regs_of(i.d)))
             elif op in ("s_cbranch_scc1", "s_cbranch_scc0", "s_branch"):
                 take = True if op == "s_branch" else (W_.scc == 1) if op == "s_cbranch_scc1" else (W_.scc == 0)
                 if take:
